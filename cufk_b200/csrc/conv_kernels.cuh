@@ -396,11 +396,11 @@ __global__ __launch_bounds__(128, kConvBackwardBlocks) void conv_backward_kernel
   }
 }
 
-// One row per chain; the state moves up by one row.
+// One row per chain; the state moves up by one row.  The kernel in front may still be writing x, the taps or the state while this one starts, so no
+// pointer is restrict: that would let the compiler read them before the wait.
 template <typename T, int W, bool SILU, bool VEC>
-__global__ __launch_bounds__(128) void conv_step_kernel(const T* __restrict__ x, int64_t x_stride, T* state, const float* __restrict__ weight,
-                                                        const float* __restrict__ bias, T* __restrict__ y, int64_t chains, int64_t width,
-                                                        int64_t columns) {
+__global__ __launch_bounds__(128) void conv_step_kernel(const T* x, int64_t x_stride, T* state, const float* weight, const float* bias, T* y, int64_t chains,
+                                                        int64_t width, int64_t columns) {
   let_next_start();
   wait_for_previous();
   const int64_t id = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;

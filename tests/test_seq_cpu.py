@@ -254,3 +254,15 @@ def test_refusals_without_a_gpu():
         seq.clip_gradients([], 1.0)
     with pytest.raises(RuntimeError, match="must not be negative"):
         seq.clip_gradients([x], -1.0)
+
+
+def test_dependent_kernels_promise_nothing_about_memory():
+    # a kernel that starts before the one in front has ended reads nothing that it declares unchanging: what that one writes changes
+    # while this one runs, and a restrict pointer would allow its reads to be made before the wait
+    for name in ("conv_kernels.cuh", "scan_kernels.cuh"):
+        source = (ROOT / "cufk_b200" / "csrc" / name).read_text()
+        kernels = re.split(r"(?=__global__ )", source)[1:]
+        waiting = [k for k in kernels if "wait_for_previous()" in k]
+        assert waiting
+        for kernel in waiting:
+            assert "__restrict__" not in kernel.split("{")[0]
