@@ -50,6 +50,12 @@ const void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr;
 void* out(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* floats(const Tensor& t) { return t.defined() ? static_cast<float*>(t.data_ptr()) : nullptr; }
 
+// The kernels write through pointers, which autograd does not see: a tensor that a call has written in place says so here, and a backward that
+// saved it refuses.  Tensors of inference mode have no version.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void check_activation(const Tensor& x, const char* name) {
   TORCH_CHECK(x.is_cuda(), name, " must be CUDA");
   const auto t = x.scalar_type();
@@ -241,6 +247,7 @@ Tensor short_conv_step(const Tensor& x, const Tensor& state, const Tensor& weigh
   check_status(cufkb_conv_step(dtype_code(x.scalar_type()), r.ptr, r.stride, state.data_ptr(), floats(w), floats(b), y.data_ptr(), x.size(0), x.size(1),
                                static_cast<int>(taps), silu, current_stream()),
                "short_conv_step");
+  written(state);
   return y;
 }
 
@@ -415,6 +422,7 @@ Tensor selective_scan_step(const Tensor& x, const Tensor& delta, const Tensor& A
   c.p.y = y.data_ptr();
   c.p.final_state = floats(state);
   check_status(cufkb_scan_step(&c.p, current_stream()), "selective_scan_step");
+  written(state);
   return y;
 }
 
@@ -523,6 +531,7 @@ Tensor clip_gradients(const std::vector<Tensor>& grads, double max_norm, double 
   Tensor norm = fresh({}, wide ? torch::kFloat64 : torch::kFloat32, first);
   check_status(cufkb_clip_gradients(arrays.data(), count, max_norm, eps, norm.data_ptr(), wide ? CUFKB_FLOAT64 : CUFKB_FLOAT32, ws.data_ptr(), bytes, current_stream()),
                "clip_gradients");
+  for (const Tensor& o : outs) written(o);
   for (auto& b : back) b.first.copy_(b.second);
   return norm;
 }
