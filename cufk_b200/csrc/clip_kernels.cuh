@@ -189,8 +189,9 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(const __grid_c
       *static_cast<float*>(norm) = static_cast<float>(total);
     }
   }
-  const double ratio = max_norm / (total + eps);
-  const double f = ratio < 1.0 || ratio != ratio ? ratio : 1.0;
+  // max_norm = inf only measures: 1 for any norm.  Compared before dividing: of inf / inf and 0 / 0 nothing is to be clipped either.
+  const double most = total + eps;
+  const double f = max_norm == INFINITY ? 1.0 : most > max_norm ? max_norm / most : most == most ? 1.0 : most;
   const int chunks = t.first[t.arrays];
   for (int chunk = chunks - 1 - static_cast<int>(blockIdx.x); chunk >= 0; chunk -= static_cast<int>(gridDim.x)) {
     with_chunk(t, chunk, [&](const auto* g, auto* out, int n) {

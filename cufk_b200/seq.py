@@ -170,13 +170,13 @@ def clip_gradients(grads: Sequence[Tensor], max_norm: float, *, out: Sequence[Te
 
     Args:
         grads: CUDA tensors of any of the four dtypes, mixed at will, on one device.  Empty ones are allowed.
-        max_norm: largest norm; ``inf`` only measures it.
+        max_norm: largest norm; ``inf`` only measures it and leaves the values as they are, whatever the norm.
         out: where the clipped gradients go, one tensor of equal shape and dtype per gradient; the gradients themselves
             when omitted (which are then not written at all where nothing needs clipping).
 
     Returns:
         The norm before clipping, a 0-d tensor on the device: float32, or float64 when some gradient is.  Squares are summed
-        in float64.  A NaN norm makes every gradient NaN, and an infinite one makes the finite ones zero.
+        in float64.  With a finite ``max_norm`` a NaN norm makes every gradient NaN, and an infinite one makes the finite ones zero.
     """
     grads = list(grads)
     return _C.clip_gradients(grads, float(max_norm), float(eps), grads if out is None else list(out))

@@ -131,8 +131,9 @@ typedef struct cufkb_grad_array {
 } cufkb_grad_array;
 
 /* norm = sqrt(sum of squares over all arrays) (double accumulation, stored as float32 or, norm_dtype =
- * CUFKB_FLOAT64, as float64); out = grad * min(1, max_norm / (norm + eps)).  All four dtypes.  `arrays` is a host
- * array, read before the call returns; the workspace is device memory. */
+ * CUFKB_FLOAT64, as float64); out = grad * min(1, max_norm / (norm + eps)), where max_norm = inf is a factor of 1
+ * for any norm.  All four dtypes.  `arrays` is a host array, read before the call returns; the workspace is device
+ * memory. */
 CUFKB_API int cufkb_clip_workspace_bytes(const cufkb_grad_array* arrays, int64_t count, size_t* bytes);
 CUFKB_API int cufkb_clip_gradients(const cufkb_grad_array* arrays, int64_t count, double max_norm, double eps, void* norm, int norm_dtype,
                                    void* workspace, size_t workspace_bytes, cufkb_stream_t stream);
