@@ -214,7 +214,8 @@ const char* cufkb_seq_status_string(int status) {
     case CUFKB_ERROR_BAD_STRIDE:
       return "strides must not be negative, nor the row strides of a scan over 2^24 elements";
     case CUFKB_ERROR_INVALID_VALUE:
-      return "a count is out of its range (taps 2 to 4, states 1 to 64, groups that divide the width, top 0 to 32)";
+      return "a count is out of its range (taps 2 to 4, states 1 to 64, groups that divide the width, top 0 to 32), or arrays of a clipping share memory that one of "
+             "them is written to";
     case CUFKB_ERROR_WORKSPACE:
       return "workspace or checkpoints are missing or too small";
     case CUFKB_ERROR_UNSUPPORTED_DTYPE:

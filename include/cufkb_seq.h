@@ -133,7 +133,8 @@ typedef struct cufkb_grad_array {
 /* norm = sqrt(sum of squares over all arrays) (double accumulation, stored as float32 or, norm_dtype =
  * CUFKB_FLOAT64, as float64); out = grad * min(1, max_norm / (norm + eps)), where max_norm = inf is a factor of 1
  * for any norm.  All four dtypes.  `arrays` is a host array, read before the call returns; the workspace is device
- * memory. */
+ * memory.  An array that is named again (equal grad, out, count and dtype) counts again in the norm and is scaled once; any other memory
+ * that is written for one array and read or written for another is refused with CUFKB_ERROR_INVALID_VALUE. */
 CUFKB_API int cufkb_clip_workspace_bytes(const cufkb_grad_array* arrays, int64_t count, size_t* bytes);
 CUFKB_API int cufkb_clip_gradients(const cufkb_grad_array* arrays, int64_t count, double max_norm, double eps, void* norm, int norm_dtype,
                                    void* workspace, size_t workspace_bytes, cufkb_stream_t stream);

@@ -266,3 +266,26 @@ def test_dependent_kernels_promise_nothing_about_memory():
         assert waiting
         for kernel in waiting:
             assert "__restrict__" not in kernel.split("{")[0]
+
+
+def test_clip_refuses_shared_memory(lib):
+    def call(*arrays):
+        list_of = (GradArray * len(arrays))(*[GradArray(*a) for a in arrays])
+        return lib.cufkb_clip_gradients(list_of, len(arrays), 1.0, 1e-6, 64, F32, 64, 1 << 30, None)
+
+    refused = [
+        [(4096, 4096, 10, F32), (4132, 4132, 10, F32)],                              # in place, one element in common
+        [(4132, 4132, 10, F32), (4096, 4096, 10, F32)],
+        [(4096, 4096, 10, F32), (4096, 4096, 9, F32)],                               # the same start
+        [(4096, 4096, 10, F32), (4096, 4096, 10, BF16)],                             # the same memory as another type
+        [(4096, 8192, 10, F32), (4200, 8228, 10, F32)],                              # results in common
+        [(4096, 8192, 10, F32), (8192, 12288, 10, F32)],                             # a result over another's gradient
+        [(8192, 12288, 10, F32), (4096, 8192, 10, F32)],
+        [(4096, 4100, 10, F32)],                                                     # over a part of its own gradient
+        [(4096, 4096, 10, F32), (4096, 8192, 10, F32)],                              # written and read again
+        [(4096, 8192, 10, F32), (4096, 4096, 10, F32)],
+        [(4096, 4096, 1000, F32), (4100, 4100, 1, F32), (4096, 4096, 1000, F32)],    # in the middle of a repeated one
+        [(4096, 4096, 10, F32), (4096, 4096, 10, F32), (4120, 4120, 1, F32)],
+    ]
+    for arrays in refused:
+        assert call(*arrays) == INVALID_VALUE, arrays
