@@ -31,15 +31,6 @@ struct ClipTable {
 };
 
 template <typename T>
-struct ClipMath {
-  using R = float;
-};
-template <>
-struct ClipMath<double> {
-  using R = double;
-};
-
-template <typename T>
 __device__ __forceinline__ double to_double(T v) {
   if constexpr (std::is_same_v<T, double>) {
     return v;
@@ -145,15 +136,24 @@ __global__ __launch_bounds__(kClipThreads) void clip_norm_kernel(const __grid_co
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
+// f = high * low.  Below float's normal range (a norm beyond 1e38 max_norm) a float factor would keep few bits or none, though what it
+// scales may well end in range; there, high = 2^-100 takes the values down first.  Elsewhere high = 1, which changes no bit.
+struct ClipFactor {
+  double f;
+  float high, low;
+  __device__ __forceinline__ explicit ClipFactor(double factor) : f(factor), high(factor < 0x1p-100 ? 0x1p-100f : 1.0f) {
+    low = static_cast<float>(factor < 0x1p-100 ? factor * 0x1p100 : factor);
+  }
+};
+
 template <typename T>
-__device__ __forceinline__ void scale_chunk(const T* g, T* out, int n, typename ClipMath<T>::R f) {
-  using R = typename ClipMath<T>::R;
+__device__ __forceinline__ void scale_chunk(const T* g, T* out, int n, const ClipFactor& c) {
   constexpr int N = 16 / sizeof(T);
   auto scaled = [&](T v) {
     if constexpr (std::is_same_v<T, double>) {
-      return v * f;
+      return v * c.f;
     } else {
-      return from_float<T>(to_float(v) * static_cast<R>(f));
+      return from_float<T>(to_float(v) * c.high * c.low);
     }
   };
   if (((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(out)) & 15) != 0) {
@@ -192,11 +192,12 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(const __grid_c
   // max_norm = inf only measures: 1 for any norm.  Compared before dividing: of inf / inf and 0 / 0 nothing is to be clipped either.
   const double most = total + eps;
   const double f = max_norm == INFINITY ? 1.0 : most > max_norm ? max_norm / most : most == most ? 1.0 : most;
+  const ClipFactor c(f);
   const int chunks = t.first[t.arrays];
   for (int chunk = chunks - 1 - static_cast<int>(blockIdx.x); chunk >= 0; chunk -= static_cast<int>(gridDim.x)) {
     with_chunk(t, chunk, [&](const auto* g, auto* out, int n) {
       if (f == 1.0 && static_cast<const void*>(g) == static_cast<const void*>(out)) return;  // in place and nothing to change
-      scale_chunk(g, out, n, static_cast<typename ClipMath<std::remove_pointer_t<decltype(out)>>::R>(f));
+      scale_chunk(g, out, n, c);
     });
   }
 }
