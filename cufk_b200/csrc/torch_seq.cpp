@@ -9,6 +9,7 @@
 #include <torch/extension.h>
 
 #include <optional>
+#include <string>
 #include <vector>
 
 #include "cufkb_seq.h"
@@ -130,6 +131,42 @@ Tensor workspace(size_t bytes, const Tensor& like) {
   return bytes == 0 ? Tensor() : fresh({static_cast<int64_t>(bytes)}, torch::kUInt8, like);
 }
 
+// Gradients that were asked for with a graph of their own (create_graph) come from kernels, which leave none.  They pass through here, so that
+// differentiating them again is an error instead of a zero.
+class OnceAutograd : public torch::autograd::Function<OnceAutograd> {
+ public:
+  // `through`: the gradients, then what they depend on
+  static tensor_list forward(AutogradContext* ctx, at::TensorList through, int64_t gradients, std::string op) {
+    ctx->saved_data["op"] = op;
+    tensor_list out;
+    for (int64_t i = 0; i < gradients; ++i) out.push_back(through[i].tensor_data());
+    return out;
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list) {
+    TORCH_CHECK(false, ctx->saved_data["op"].toStringRef(), " can be differentiated only once");
+  }
+};
+
+tensor_list differentiated_once(tensor_list grads, const tensor_list& outputs, const tensor_list& inputs, const char* op) {
+  if (!at::GradMode::is_enabled()) return grads;
+  tensor_list through;
+  for (const Tensor& t : grads) {
+    if (t.defined()) through.push_back(t);
+  }
+  const int64_t count = static_cast<int64_t>(through.size());
+  for (const tensor_list* list : {&outputs, &inputs}) {
+    for (const Tensor& t : *list) {
+      if (t.defined()) through.push_back(t);
+    }
+  }
+  const tensor_list marked = OnceAutograd::apply(at::TensorList(through), count, std::string(op));
+  size_t next = 0;
+  for (Tensor& t : grads) {
+    if (t.defined()) t = marked[next++];
+  }
+  return grads;
+}
+
 // ---------------------------------------------------------------------------------------------
 // short causal convolution
 // ---------------------------------------------------------------------------------------------
@@ -222,7 +259,7 @@ class ConvAutograd : public torch::autograd::Function<ConvAutograd> {
     c.p.grad_bias = floats(gb);
     c.p.grad_initial_state = out(gi);
     check_status(cufkb_conv_backward(&c.p, current_stream()), "short_conv backward");
-    return {gx, gw, bias.defined() ? gb : Tensor(), Tensor(), gi, Tensor(), Tensor()};
+    return differentiated_once({gx, gw, bias.defined() ? gb : Tensor(), Tensor(), gi, Tensor(), Tensor()}, grads, saved, "short_conv");
   }
 };
 
@@ -392,7 +429,7 @@ class ScanAutograd : public torch::autograd::Function<ScanAutograd> {
     c.p.grad_delta_bias = floats(gbias);
     c.p.grad_initial_state = floats(gi);
     check_status(cufkb_scan_backward(&c.p, current_stream()), "selective_scan backward");
-    return {gx, gd, gA, gB, gC, gD, gz, gbias, Tensor(), gi, Tensor(), Tensor(), Tensor()};
+    return differentiated_once({gx, gd, gA, gB, gC, gD, gz, gbias, Tensor(), gi, Tensor(), Tensor(), Tensor()}, grads, saved, "selective_scan");
   }
 };
 
@@ -484,7 +521,7 @@ class LogprobsAutograd : public torch::autograd::Function<LogprobsAutograd> {
     check_status(cufkb_token_logprobs_backward(dtype_code(logits.scalar_type()), l.ptr, l.stride, saved[1].data_ptr<int64_t>(), floats(saved[2]), floats(saved[3]),
                                                floats(gl), floats(gh), g.data_ptr(), rows, logits.size(-1), current_stream()),
                  "token_logprobs backward");
-    return {g, Tensor(), Tensor()};
+    return differentiated_once({g, Tensor(), Tensor()}, grads, saved, "token_logprobs");
   }
 };
 

@@ -14,6 +14,8 @@ of a wider projection is read in place).  They are float32, float16 or bfloat16,
 output; parameters, scan states and their gradients are float32.  ``chain_points`` stays on the device and is not
 checked there beyond what keeps every access inside the arrays: it must start at 0 and not decrease.
 
+Gradients are first derivatives: under ``create_graph`` they are the same, and differentiating them again is an error.
+
 All calls run on the current stream and never synchronise with the host.  Sums over rows, channels and arrays are taken in an
 order that depends on sizes alone, so results repeat bit by bit.
 """
