@@ -63,6 +63,13 @@ void check_activation(const Tensor& x, const char* name) {
   TORCH_CHECK(t == torch::kFloat32 || t == torch::kFloat16 || t == torch::kBFloat16, name, " must be float32, float16, or bfloat16");
 }
 
+bool asks_gradient(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+void refuse_gradients(std::initializer_list<Tensor> inputs, const char* op) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor& t : inputs) TORCH_CHECK(!asks_gradient(t), op, " takes no gradients");
+}
+
 void check_like(const Tensor& x, const Tensor& ref, const char* name, const char* ref_name) {
   TORCH_CHECK(x.is_cuda() && x.device() == ref.device(), name, " must be CUDA, on the device of ", ref_name);
   TORCH_CHECK(x.scalar_type() == ref.scalar_type(), name, " must have the dtype of ", ref_name);
@@ -276,7 +283,7 @@ Tensor short_conv_step(const Tensor& x, const Tensor& state, const Tensor& weigh
   TORCH_CHECK(taps >= CUFKB_MIN_TAPS && taps <= CUFKB_MAX_TAPS, "weight must have ", CUFKB_MIN_TAPS, " to ", CUFKB_MAX_TAPS, " taps");
   TORCH_CHECK(state.sizes() == at::IntArrayRef({x.size(0), taps - 1, x.size(1)}) && state.is_contiguous(),
               "state must be contiguous, of shape (chains, taps - 1, width)");
-  TORCH_CHECK(!at::GradMode::is_enabled() || !(x.requires_grad() || state.requires_grad() || weight.requires_grad()), "short_conv_step takes no gradients");
+  refuse_gradients({x, state, weight, get(bias)}, "short_conv_step");
   const Tensor w = check_float(weight, {x.size(1), taps}, x, "weight"), b = check_float(get(bias), {x.size(1)}, x, "bias");
   const c10::cuda::CUDAGuard guard(x.device());
   const Rows r = rows_of(x);
@@ -435,9 +442,9 @@ class ScanAutograd : public torch::autograd::Function<ScanAutograd> {
 
 tensor_list selective_scan(const Tensor& x, const Tensor& delta, const Tensor& A, const Tensor& B, const Tensor& C, const OptTensor& D, const OptTensor& z,
                            const OptTensor& bias, const OptTensor& points, const OptTensor& initial, bool softplus, bool keep) {
-  auto asks = [](const OptTensor& t) { return t.has_value() && t->defined() && t->requires_grad(); };
   const bool train = at::GradMode::is_enabled() && (x.requires_grad() || delta.requires_grad() || A.requires_grad() || B.requires_grad() ||
-                                                    C.requires_grad() || asks(D) || asks(z) || asks(bias) || asks(initial));
+                                                    C.requires_grad() || asks_gradient(get(D)) || asks_gradient(get(z)) ||
+                                                    asks_gradient(get(bias)) || asks_gradient(get(initial)));
   return ScanAutograd::apply(x, delta, A, B, C, D, z, bias, points, initial, softplus, keep, train);
 }
 
@@ -445,8 +452,7 @@ Tensor selective_scan_step(const Tensor& x, const Tensor& delta, const Tensor& A
                            const OptTensor& z, const OptTensor& bias, bool softplus) {
   check_activation(x, "x");
   TORCH_CHECK(x.dim() == 2, "x must have shape (chains, width)");
-  TORCH_CHECK(!at::GradMode::is_enabled() || !(x.requires_grad() || delta.requires_grad() || A.requires_grad() || state.requires_grad()),
-              "selective_scan_step takes no gradients");
+  refuse_gradients({x, delta, A, B, C, state, get(D), get(z), get(bias)}, "selective_scan_step");
   Layout l;
   l.rows = l.chains = x.size(0);
   l.width = x.size(1);
