@@ -49,7 +49,7 @@ struct ScanArgs {
   int softplus;
   int width, group_width, states, blocks_per_group, blocks;  // blocks: of channels, over all groups
   const T *x, *delta, *z;
-  int x_stride, delta_stride, z_stride;  // at most 2^24: the rows of a tile are addressed with 32 bits from its first
+  int x_stride, delta_stride, z_stride;  // at most 2^24, but for a step: the rows of a tile are addressed with 32 bits from its first
   const float* A;
   const T *B, *C;
   int B_stride, C_stride;

@@ -212,7 +212,7 @@ const char* cufkb_seq_status_string(int status) {
     case CUFKB_ERROR_SHAPE_LIMITS:
       return "a size is negative or too large, or rows do not split into equal chains";
     case CUFKB_ERROR_BAD_STRIDE:
-      return "strides must not be negative, nor the row strides of a scan over 2^24 elements";
+      return "strides must not be negative, nor the row strides of a scan over 2^24 elements (of its step 2^31 - 1)";
     case CUFKB_ERROR_INVALID_VALUE:
       return "a count is out of its range (taps 2 to 4, states 1 to 64, groups that divide the width, top 0 to 32), or arrays of a clipping share memory that one of "
              "them is written to";

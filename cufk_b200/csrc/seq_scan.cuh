@@ -62,8 +62,6 @@ inline ScanPlan scan_plan(const cufkb_scan_params& q, bool backward) {
   return p;
 }
 
-constexpr int64_t kMostStride = int64_t{1} << 24;  // elements between rows
-
 struct ScanSpace {
   size_t piece_state, piece_dt, partial_bc, partial_A, partial_d, total;
 };
@@ -87,7 +85,7 @@ inline ScanSpace scan_space(const cufkb_scan_params& q, const ScanPlan& p, bool 
   return s;
 }
 
-inline int scan_check(const cufkb_scan_params& q) {
+inline int scan_check(const cufkb_scan_params& q, int64_t most_stride = CUFKB_MAX_SCAN_STRIDE) {
   if (int st = check_activation_dtype(q.dtype)) return st;
   if (int st = check_rows(q.rows, q.chains, q.width, q.chain_points)) return st;
   if (q.states < 1 || q.states > CUFKB_MAX_STATES || q.groups < 1 || q.width % q.groups != 0) return CUFKB_ERROR_INVALID_VALUE;
@@ -97,7 +95,7 @@ inline int scan_check(const cufkb_scan_params& q) {
   }
   const int64_t row_strides[] = {q.x_stride, q.delta_stride, q.z_stride, q.B_stride, q.C_stride, q.grad_y_stride};
   for (int64_t stride : row_strides) {
-    if (stride > kMostStride) return CUFKB_ERROR_BAD_STRIDE;
+    if (stride > most_stride) return CUFKB_ERROR_BAD_STRIDE;
   }
   const size_t e = element_size(q.dtype);
   const void* const ptrs2[] = {q.x, q.delta, q.z, q.B, q.C, static_cast<const void*>(q.y), q.grad_y, static_cast<const void*>(q.grad_x),

@@ -111,7 +111,7 @@ int cufkb_scan_step(const cufkb_scan_params* params, cufkb_stream_t stream) {
   q.rows = q.chains;
   q.chain_points = nullptr;
   q.workspace = nullptr;
-  if (int st = scan_check(q)) return st;
+  if (int st = scan_check(q, CUFKB_MAX_STEP_STRIDE)) return st;
   if (q.width == 0 || q.chains == 0) return CUFKB_SUCCESS;
   if (int st = scan_check_inputs(q)) return st;
   if (q.y == nullptr || q.final_state == nullptr) return CUFKB_ERROR_NULL_POINTER;

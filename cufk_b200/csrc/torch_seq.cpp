@@ -84,23 +84,28 @@ Tensor check_float(const Tensor& x, at::IntArrayRef shape, const Tensor& ref, co
   return x.contiguous();
 }
 
-// Rows of a (..., width) activation as (rows, width) with one row stride; a copy only where there is none.
+// The widest row strides that a scan and its step walk (cufkb_scan_params); rows further apart are copied.
+constexpr int64_t kScanStride = CUFKB_MAX_SCAN_STRIDE, kStepStride = CUFKB_MAX_STEP_STRIDE;
+
+// Rows of a (..., width) activation as (rows, width) with one row stride of at most `most`; a copy only where there is none.
 struct Rows {
   Tensor kept;
   const void* ptr = nullptr;
   int64_t stride = 0;
 };
 
-Rows rows_of(const Tensor& x) {
+Rows rows_of(const Tensor& x, int64_t most = INT64_MAX) {
   Rows r;
-  r.kept = x;
-  const int64_t d = x.dim();
-  bool flat = x.numel() == 0 || x.size(d - 1) <= 1 || x.stride(d - 1) == 1;
+  const int64_t d = x.dim(), width = x.size(d - 1), rows = d == 3 ? x.size(0) * x.size(1) : x.size(0);
+  bool flat = x.numel() == 0 || width <= 1 || x.stride(d - 1) == 1;
   if (flat && d == 3 && x.size(0) > 1 && x.size(1) > 1) flat = x.stride(0) == x.size(1) * x.stride(1);
-  if (!flat) r.kept = x.contiguous();
+  auto stride_of = [&](const Tensor& t) {
+    if (rows <= 1 || width == 0) return width;  // never used
+    return (d == 3 && t.size(1) <= 1) ? t.stride(0) : t.stride(d - 2);
+  };
+  r.kept = flat && stride_of(x) <= most ? x : x.contiguous();
   r.ptr = r.kept.data_ptr();
-  r.stride = (d == 3 && r.kept.size(1) <= 1) ? r.kept.stride(0) : r.kept.stride(d - 2);
-  if (r.kept.size(d - 1) == 0) r.stride = 0;
+  r.stride = stride_of(r.kept);
   return r;
 }
 
@@ -305,7 +310,8 @@ struct ScanCall {
 };
 
 // (rows, states), (rows, groups, states), or the same with (chains, length) in the place of rows: pointer and strides
-Tensor bc_rows(const Tensor& t, const Tensor& x, const Layout& l, int64_t states, int64_t& groups, int64_t& stride, int64_t& group_stride, const char* name) {
+Tensor bc_rows(const Tensor& t, const Tensor& x, const Layout& l, int64_t states, int64_t most, int64_t& groups, int64_t& stride, int64_t& group_stride,
+               const char* name) {
   check_like(t, x, name, "x");
   const int64_t lead = x.dim() - 1;
   TORCH_CHECK(t.dim() == lead + 1 || t.dim() == lead + 2, name, " must have shape (rows, states) or (rows, groups, states), rows as in x");
@@ -315,14 +321,18 @@ Tensor bc_rows(const Tensor& t, const Tensor& x, const Layout& l, int64_t states
   TORCH_CHECK(groups >= 1 && l.width % groups == 0, name, ": the groups must divide the width");
   bool flat = states <= 1 || t.stride(-1) == 1;
   if (flat && lead == 2 && t.size(0) > 1 && t.size(1) > 1) flat = t.stride(0) == t.size(1) * t.stride(1);
-  const Tensor kept = flat ? t : t.contiguous();
-  stride = (lead == 2 && kept.size(1) <= 1) ? kept.stride(0) : kept.stride(lead - 1);
+  auto stride_of = [&](const Tensor& v) {
+    if (l.rows <= 1) return states * groups;  // never used
+    return (lead == 2 && v.size(1) <= 1) ? v.stride(0) : v.stride(lead - 1);
+  };
+  const Tensor kept = flat && stride_of(t) <= most ? t : t.contiguous();
+  stride = stride_of(kept);
   group_stride = kept.dim() == lead + 2 ? kept.stride(lead) : 0;
   return kept;
 }
 
 ScanCall scan_call(const Tensor& x, const Tensor& delta, const Tensor& A, const Tensor& B, const Tensor& C, const Tensor& D, const Tensor& z,
-                   const Tensor& bias, const Tensor& points, const Tensor& initial, bool softplus, const Layout& l) {
+                   const Tensor& bias, const Tensor& points, const Tensor& initial, bool softplus, const Layout& l, int64_t most = kScanStride) {
   ScanCall c;
   check_like(delta, x, "delta", "x");
   TORCH_CHECK(delta.sizes() == x.sizes(), "delta must have the shape of x");
@@ -337,13 +347,13 @@ ScanCall scan_call(const Tensor& x, const Tensor& delta, const Tensor& A, const 
   c.D = check_float(D, {l.width}, x, "D");
   c.bias = check_float(bias, {l.width}, x, "delta_bias");
   int64_t groups = 1, groups_c = 1;
-  c.B = bc_rows(B, x, l, states, groups, c.p.B_stride, c.p.B_group_stride, "B");
-  c.C = bc_rows(C, x, l, states, groups_c, c.p.C_stride, c.p.C_group_stride, "C");
+  c.B = bc_rows(B, x, l, states, most, groups, c.p.B_stride, c.p.B_group_stride, "B");
+  c.C = bc_rows(C, x, l, states, most, groups_c, c.p.C_stride, c.p.C_group_stride, "C");
   TORCH_CHECK(groups == groups_c, "B and C must have the same groups");
   c.initial = check_float(initial, {l.chains, l.width, states}, x, "initial_state");
-  c.x = rows_of(x);
-  c.delta = rows_of(delta);
-  if (z.defined()) c.z = rows_of(z);
+  c.x = rows_of(x, most);
+  c.delta = rows_of(delta, most);
+  if (z.defined()) c.z = rows_of(z, most);
   c.p.dtype = dtype_code(x.scalar_type());
   c.p.softplus = softplus;
   c.p.rows = l.rows;
@@ -405,7 +415,7 @@ class ScanAutograd : public torch::autograd::Function<ScanAutograd> {
     const c10::cuda::CUDAGuard guard(x.device());
     const Tensor gy = grads[0].defined() ? grads[0] : torch::zeros(x.sizes(), x.options());
     check_like(gy, x, "grad_y", "x");
-    const Rows g = rows_of(gy);
+    const Rows g = rows_of(gy, kScanStride);
     c.p.grad_y = g.ptr;
     c.p.grad_y_stride = g.stride;
     Tensor gs;
@@ -456,7 +466,7 @@ Tensor selective_scan_step(const Tensor& x, const Tensor& delta, const Tensor& A
   Layout l;
   l.rows = l.chains = x.size(0);
   l.width = x.size(1);
-  ScanCall c = scan_call(x, delta, A, B, C, get(D), get(z), get(bias), Tensor(), Tensor(), softplus, l);
+  ScanCall c = scan_call(x, delta, A, B, C, get(D), get(z), get(bias), Tensor(), Tensor(), softplus, l, kStepStride);
   TORCH_CHECK(state.is_cuda() && state.device() == x.device() && state.scalar_type() == torch::kFloat32 && state.is_contiguous() &&
                   state.sizes() == at::IntArrayRef({l.chains, l.width, c.p.states}),
               "state must be contiguous float32 of shape (chains, width, states), on the device of x");

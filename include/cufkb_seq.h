@@ -31,6 +31,8 @@ extern "C" {
 #define CUFKB_MIN_TAPS 2
 #define CUFKB_MAX_TAPS 4
 #define CUFKB_MAX_TOP 32
+#define CUFKB_MAX_SCAN_STRIDE (1 << 24) /* elements between the rows of a scan */
+#define CUFKB_MAX_STEP_STRIDE 0x7fffffff /* and of its single-row step */
 
 /* Short causal convolution, one filter per channel: pre[t] = bias + sum_k weight[:, k] x[t-taps+1+k],
  * y = pre sigmoid(pre) (silu != 0) or pre.  Rows before a chain's start are initial_state's taps-1 rows,
@@ -77,7 +79,7 @@ typedef struct cufkb_scan_params {
   int dtype, softplus;
   int64_t rows, chains, width, groups, states;
   const int64_t* chain_points; /* (chains+1) or NULL */
-  const void *x, *delta, *z;   /* (rows, width), row strides below; z may be NULL */
+  const void *x, *delta, *z;   /* (rows, width), row strides below (all row strides at most CUFKB_MAX_SCAN_STRIDE); z may be NULL */
   int64_t x_stride, delta_stride, z_stride;
   const float* A;              /* (width, states) */
   const void *B, *C;           /* (rows, groups, states): row and group strides, states contiguous */
@@ -104,7 +106,7 @@ CUFKB_API int cufkb_scan_forward(const cufkb_scan_params* params, cufkb_stream_t
 CUFKB_API int cufkb_scan_backward(const cufkb_scan_params* params, cufkb_stream_t stream);
 
 /* One row per chain (rows = chains, chain_points, checkpoints and workspace ignored): `final_state`
- * (chains, width, states) is read and updated in place. */
+ * (chains, width, states) is read and updated in place.  Row strides are at most CUFKB_MAX_STEP_STRIDE. */
 CUFKB_API int cufkb_scan_step(const cufkb_scan_params* params, cufkb_stream_t stream);
 
 /* Per row of logits (rows, tokens_count), row stride logits_stride: logp of the given token, the entropy
