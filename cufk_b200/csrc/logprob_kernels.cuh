@@ -337,9 +337,9 @@ struct RowGrad {
     log_s = log_sum[2 * r + 1];
     c = fmaf(h, entropy[r], g);
     if (m == -INFINITY) {
-      // no token is possible: p = 0 everywhere, and no gradient
+      // no token is possible: p = 0 everywhere, and no gradient, whatever comes back (NaN from p log p, say)
       m = INFINITY;
-      g = 0.0f;
+      g = h = c = 0.0f;
     }
   }
   // a block from id `first` on
