@@ -17,6 +17,8 @@
 // that a piece starts from with one multiply-add per earlier piece.  The backward does the same from the chain's end.
 #pragma once
 
+#include <cfloat>
+
 #include "seq_common.cuh"
 
 namespace cufkb_seq {
@@ -109,7 +111,7 @@ struct Place {
 
 // The thread's states of its channels, out of (width, states) floats.
 template <int KN, int KC>
-__device__ __forceinline__ void load_states(Pair (&h)[KC][KN / 2], const float* base, int64_t channel, int left, int states, int n0, float scale) {
+__device__ __forceinline__ void load_states(Pair (&h)[KC][KN / 2], const float* base, int64_t channel, int left, int states, int n0) {
 #pragma unroll
   for (int c = 0; c < KC; ++c) {
 #pragma unroll
@@ -118,9 +120,27 @@ __device__ __forceinline__ void load_states(Pair (&h)[KC][KN / 2], const float* 
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int n = n0 + 2 * i + k;
-        v[k] = (base != nullptr && c < left && n < states) ? base[(channel + c) * states + n] * scale : 0.0f;
+        v[k] = (base != nullptr && c < left && n < states) ? base[(channel + c) * states + n] : 0.0f;
       }
       h[c][i] = pair(v[0], v[1]);
+    }
+  }
+}
+// A log2(e), so that exp(dt A) is 2 to the power of dt times it.  -inf (of A, or of the product) becomes the lowest finite number: its
+// exponential is 0 for any dt a row has, and 1 for the dt = 0 of the places behind a chain's end, where -inf would make NaN.
+__device__ __forceinline__ float decay_of(float a) {
+  const float v = a * kLog2e;
+  return v < -FLT_MAX ? -FLT_MAX : v;
+}
+template <int KN, int KC>
+__device__ __forceinline__ void load_decays(Pair (&A2)[KC][KN / 2], const float* A, int64_t channel, int left, int states, int n0) {
+  load_states<KN, KC>(A2, A, channel, left, states, n0);
+#pragma unroll
+  for (int c = 0; c < KC; ++c) {
+#pragma unroll
+    for (int i = 0; i < KN / 2; ++i) {
+      const float2 v = halves(A2[c][i]);
+      A2[c][i] = pair(decay_of(v.x), decay_of(v.y));
     }
   }
 }
@@ -348,11 +368,11 @@ __global__ __launch_bounds__(kScanThreads, kForwardBlocks) void scan_forward_ker
   const float bias = p.bias != nullptr ? p.bias[own] : 0.0f, D = !LOCAL && p.D != nullptr ? p.D[own] : 0.0f;
 
   Pair A2[KC][kPairs], h[KC][kPairs];
-  load_states<KN, KC>(A2, p.A, channel, left, p.states, at.n0, kLog2e);
+  load_decays<KN, KC>(A2, p.A, channel, left, p.states, at.n0);
   if (LOCAL) {
-    load_states<KN, KC>(h, nullptr, channel, left, p.states, at.n0, 1.0f);
+    load_states<KN, KC>(h, nullptr, channel, left, p.states, at.n0);
   } else {
-    load_states<KN, KC>(h, p.initial != nullptr ? p.initial + piece.chain * p.width * p.states : nullptr, channel, left, p.states, at.n0, 1.0f);
+    load_states<KN, KC>(h, p.initial != nullptr ? p.initial + piece.chain * p.width * p.states : nullptr, channel, left, p.states, at.n0);
     if (piece.index > 0) wait_for_previous();
     over_pieces<T, KN, KC, NP>(h, p, piece.chain_first, p.length, piece.index, channel, left, at.n0, A2);
   }
@@ -505,7 +525,7 @@ __global__ __launch_bounds__(kScanThreads, LOCAL ? 4 : kBackwardBlocks) void sca
   const float bias = p.bias != nullptr ? p.bias[own] : 0.0f, D = p.D != nullptr ? p.D[own] : 0.0f;
 
   Pair A2[KC][kPairs], dA[KC][kPairs] = {};
-  load_states<KN, KC>(A2, p.A, channel, left, p.states, at.n0, kLog2e);
+  load_decays<KN, KC>(A2, p.A, channel, left, p.states, at.n0);
   float dD = 0.0f, dbias = 0.0f;
   if constexpr (!LOCAL) {
     if (at.idle()) {
@@ -563,10 +583,10 @@ __global__ __launch_bounds__(kScanThreads, LOCAL ? 4 : kBackwardBlocks) void sca
     }
     Pair R[KC][kPairs];
     if (LOCAL) {
-      load_states<KN, KC>(R, nullptr, channel, left, p.states, at.n0, 1.0f);
+      load_states<KN, KC>(R, nullptr, channel, left, p.states, at.n0);
     } else {
       // what the chain's end hands back, through the pieces behind this one
-      load_states<KN, KC>(R, p.grad_final != nullptr ? p.grad_final + piece.chain * p.width * p.states : nullptr, channel, left, p.states, at.n0, 1.0f);
+      load_states<KN, KC>(R, p.grad_final != nullptr ? p.grad_final + piece.chain * p.width * p.states : nullptr, channel, left, p.states, at.n0);
       const int64_t behind = pieces_of(piece.chain_end - piece.chain_first, p.length) - 1 - piece.index;
       over_pieces<T, KN, KC, NP>(R, p, piece.chain_first + (piece.index + behind - 1) * p.length, -p.length, behind, channel, left, at.n0, A2);
     }
@@ -831,7 +851,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(ScanArgs<T> p) 
   const int own = mine ? d : 0;
   Block<float, kPer> A = load_block<float, kPer, VEC>(p.A + static_cast<int64_t>(own) * p.states + n0, left);
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) A.v[i] *= kLog2e;
+  for (int i = 0; i < kPer; ++i) A.v[i] = decay_of(A.v[i]);
   const float bias = p.bias != nullptr ? p.bias[own] : 0.0f, D = p.D != nullptr ? p.D[own] : 0.0f;
   const T *bp = p.B + g * p.B_group_stride + n0, *cp = p.C + g * p.C_group_stride + n0;
   const int64_t next = static_cast<int64_t>(p.width) * p.states;
