@@ -303,7 +303,7 @@ __device__ __forceinline__ void over_pieces(Pair (&h)[KC][KN / 2], const ScanArg
       for (int c = 0; c < KC; ++c) {
         const Pair s = pair(sum[j][c], sum[j][c]);
 #pragma unroll
-        for (int i = 0; i < KN / 2; ++i) h[c][i] = fma2(exp2_pair(mul2(s, A2[c][i])), h[c][i], e[j][c][i]);
+        for (int i = 0; i < KN / 2; ++i) h[c][i] = fma2(decay2(s, A2[c][i]), h[c][i], e[j][c][i]);
       }
     }
   }
@@ -417,7 +417,7 @@ __global__ __launch_bounds__(kScanThreads, kForwardBlocks) void scan_forward_ker
         for (int c = 0; c < KC; ++c) {
           const Pair dt = pair(du.v[c].x, du.v[c].x), u = pair(du.v[c].y, du.v[c].y);
 #pragma unroll
-          for (int i = 0; i < kPairs; ++i) h[c][i] = fma2(exp2_pair(mul2(dt, A2[c][i])), h[c][i], mul2(u, b[i]));
+          for (int i = 0; i < kPairs; ++i) h[c][i] = fma2(decay2(dt, A2[c][i]), h[c][i], mul2(u, b[i]));
         }
         if constexpr (!LOCAL) {
           Pair cc[kPairs];
@@ -631,7 +631,7 @@ __global__ __launch_bounds__(kScanThreads, LOCAL ? 4 : kBackwardBlocks) void sca
           for (int c = 0; c < KC; ++c) {
             const Pair dt = pair(du.v[c].x, du.v[c].x), dyp = pair(dy.v[c], dy.v[c]);
 #pragma unroll
-            for (int i = 0; i < kPairs; ++i) R[c][i] = mul2(exp2_pair(mul2(dt, A2[c][i])), fma2(cc[i], dyp, R[c][i]));
+            for (int i = 0; i < kPairs; ++i) R[c][i] = mul2(decay2(dt, A2[c][i]), fma2(cc[i], dyp, R[c][i]));
           }
         }
         __syncthreads();
@@ -654,7 +654,7 @@ __global__ __launch_bounds__(kScanThreads, LOCAL ? 4 : kBackwardBlocks) void sca
               Pair y = 0;
 #pragma unroll
               for (int i = 0; i < kPairs; ++i) {
-                ah[t][c][i] = mul2(exp2_pair(mul2(dt, A2[c][i])), h[c][i]);
+                ah[t][c][i] = mul2(decay2(dt, A2[c][i]), h[c][i]);
                 h[c][i] = fma2(u, b[i], ah[t][c][i]);
                 dC[i] = c ? fma2(h[c][i], dyp, dC[i]) : mul2(h[c][i], dyp);
                 y = i ? fma2(h[c][i], cc[i], y) : mul2(h[c][i], cc[i]);
@@ -702,7 +702,7 @@ __global__ __launch_bounds__(kScanThreads, LOCAL ? 4 : kBackwardBlocks) void sca
                 ma = i ? fma2(m, A2[c][i], ma) : mul2(m, A2[c][i]);
                 gb = i ? fma2(gr, b[i], gb) : mul2(gr, b[i]);
                 dB[i] = c ? fma2(gr, u, dB[i]) : mul2(gr, u);
-                R[c][i] = mul2(exp2_pair(mul2(dt, A2[c][i])), gr);  // a_t once more: cheaper than its registers
+                R[c][i] = mul2(decay2(dt, A2[c][i]), gr);  // a_t once more: cheaper than its registers
               }
               sa[(t % kBatch) * KC + c] = sum_pair(ma);
               sb[(t % kBatch) * KC + c] = sum_pair(gb);
@@ -880,7 +880,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(ScanArgs<T> p) 
       y[k] = 0.0f;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        h[k].v[i] = fmaf(exp2_fast(dk * A.v[i]), h[k].v[i], uk * to_float(b[k].v[i]));
+        h[k].v[i] = fmaf(decay(dk, A.v[i]), h[k].v[i], uk * to_float(b[k].v[i]));
         y[k] = i < left ? fmaf(h[k].v[i], to_float(c[k].v[i]), y[k]) : y[k];
       }
       if (k < real) store_block<float, kPer, VEC>(state + k * next, h[k], left);

@@ -120,6 +120,17 @@ __device__ __forceinline__ Pair exp2_pair(Pair v) {
   const float2 f = halves(v);
   return pair(exp2_fast(f.x), exp2_fast(f.y));
 }
+// A decay, exp(dt A) = 2^(dt A2) with A2 = A log2(e).  The exponential unit's results are low in the mean, by 0.5e-8 for exponents of -2^-8 and
+// nearer to 0, by 1.8e-8 to 2.7e-8 from -2^-7 to -2^-4 (about an rms of 3e-8 to 4e-8; correct rounding would have 1.7e-8 and no mean), and a recurrence
+// multiplies one decay per row: rounding averages out, a mean adds up.  2^-26 in the exponent raises the result by 1.03e-8: half of
+// the mean where it is large, and no more off above than below where it is small.  It costs nothing, the product becomes an fma, and
+// exponents of 0 still give 1.  Against 64 bits, relative: the gradient of A at 8192 x 2048 x 16 (bfloat16) 1.35e-6 without it and 0.77e-6
+// with it, the last state at 16384 x 1024 x 16 5.3e-7 and 3.0e-7.  A correctly rounded exponential, made in 64 bits,
+// gives 0.26e-6 and 1.5e-7, at four times the time.
+constexpr float kDecayMean = 1.4901161e-8f;
+__device__ __forceinline__ float decay(float dt, float A2) { return exp2_fast(fmaf(dt, A2, kDecayMean)); }
+__device__ __forceinline__ Pair decay2(Pair dt, Pair A2) { return exp2_pair(fma2(dt, A2, pair(kDecayMean, kDecayMean))); }
+
 __device__ __forceinline__ float sum_pair(Pair v) {
   const float2 f = halves(v);
   return f.x + f.y;
