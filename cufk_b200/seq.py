@@ -10,14 +10,18 @@ them.  Each is a hand-written sm_100a kernel behind the C ABI of ``include/cufkb
 Rows and chains.  Activations are ``(rows, width)`` with ``chain_points``, the ``(chains + 1,)`` int64 offsets of the
 chains on the device (a chain may be empty; rows past the last offset are padding, whose results and gradients are zero);
 ``(chains, length, width)``; or ``(rows, width)`` for one chain.  Columns are contiguous, rows may have any stride (a slice
-of a wider projection is read in place).  They are float32, float16 or bfloat16, computed in float32 and rounded once on
+of a wider projection is read in place; rows of a scan that are more than 2^24 elements apart are copied first).  They are float32, float16 or bfloat16, computed in float32 and rounded once on
 output; parameters, scan states and their gradients are float32.  ``chain_points`` stays on the device and is not
 checked there beyond what keeps every access inside the arrays: it must start at 0 and not decrease.
 
 Gradients are first derivatives: under ``create_graph`` they are the same, and differentiating them again is an error.
 
 All calls run on the current stream and never synchronise with the host.  Sums over rows, channels and arrays are taken in an
-order that depends on sizes alone, so results repeat bit by bit.
+order that depends on sizes and on the alignment of the arrays alone, so results of the same call repeat bit by bit.  Exponentials are the
+hardware's, good to 2^-22; in chains of up to 16384 rows the last states and the gradient of A were off by less than 1e-6 of their norms.
+
+These are plain functions of the extension, not ``torch.library`` operators like those of ``cufk_b200.ops``: ``torch.compile`` breaks its
+graph at them.  CUDA graphs capture them.
 """
 
 from __future__ import annotations
@@ -76,7 +80,7 @@ def short_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Tensor | Non
     r"""One more row of every chain: ``short_conv`` of ``x`` ``(chains, width)`` after the rows in ``state``.
 
     ``state``, ``(chains, taps - 1, width)`` contiguous in the dtype of ``x``, is updated in place: its oldest row leaves, ``x`` is
-    its newest.  No gradients.
+    its newest.  No gradients: with grad mode on, an argument that asks for one is refused.
     """
     return _C.short_conv_step(x, state, weight, bias, silu)
 
@@ -115,7 +119,8 @@ def selective_scan(
 
     Returns:
         ``y`` in the shape and dtype of ``x``, or ``(y, state)``.  Gradients flow to every floating argument, from both results.
-        When one is asked for, the forward keeps the state every 8 rows (``width * states / 2`` bytes per row, states rounded up to 8, 16, 32 or 64).
+        When one is asked for, the forward keeps the state every 8 rows (``width * states / 2`` bytes per row, states rounded up to 8, 16, 32 or 64), and
+        the backward's workspace holds ``width * states**2 / 128`` more (partial sums for B and C).
     """
     out = _C.selective_scan(x, delta, A, B, C, D, z, delta_bias, chain_points, initial_state, delta_softplus, return_state)
     return (out[0], out[1]) if return_state else out[0]
@@ -137,7 +142,7 @@ def selective_scan_step(
     r"""One more row of every chain: ``selective_scan`` of ``(chains, width)`` rows from ``state``.
 
     ``B`` and ``C`` are ``(chains, states)`` or ``(chains, groups, states)``.  ``state``, ``(chains, width, states)`` contiguous
-    float32, is updated in place.  No gradients.
+    float32, is updated in place.  No gradients: with grad mode on, an argument that asks for one is refused.
     """
     return _C.selective_scan_step(x, delta, A, B, C, state, D, z, delta_bias, delta_softplus)
 
