@@ -177,7 +177,9 @@ __device__ __forceinline__ void cp_async_wait_group() {
 // global-memory access: griddepcontrol.wait returns once the previous grid has completed and its
 // writes are visible (the ordering of a plain launch; a no-op when the launch did not allow the
 // overlap), and launch_dependents then lets the next kernel in the stream be scheduled once every
-// CTA of this grid has started.  The saving is the launch latency between dependent kernels.
+// CTA of this grid has started.  The saving is the launch latency between dependent kernels.  Inputs of
+// such kernels are not restrict: the previous grid may write them while this one starts, and const with
+// restrict would let the compiler read them before the wait.
 __device__ __forceinline__ void enter_after_previous_grid() {
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");

@@ -639,7 +639,7 @@ __global__ void __launch_bounds__(kMaxWarps* kWarp)
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kMaxWarps* kWarp) block_backward_kernel(BlockArgs<T> args, const T* __restrict__ grad_xyz, T* __restrict__ grad_lengths,
+__global__ void __launch_bounds__(kMaxWarps* kWarp) block_backward_kernel(BlockArgs<T> args, const T* grad_xyz, T* __restrict__ grad_lengths,
                                                                          T* __restrict__ grad_angles, T* __restrict__ grad_dihedrals, ChainGeometry geo) {
   enter_after_previous_grid();
   using R = typename ComputeOf<T>::type;
@@ -836,7 +836,7 @@ __device__ __forceinline__ void backward_xyz_staged(ChainViews<T>& cv, CtaExchan
 // sin^2 theta < 1e-2 (bond angle within ~6 degrees of 0 or pi), or when a value is not finite.
 template <typename T>
 __global__ void __launch_bounds__(kMaxWarps* kWarp)
-    block_backward_xyz_kernel(BlockArgs<T> args, const T* __restrict__ xyz, const T* __restrict__ grad_xyz, T* __restrict__ grad_lengths,
+    block_backward_xyz_kernel(BlockArgs<T> args, const T* xyz, const T* grad_xyz, T* __restrict__ grad_lengths,
                               T* __restrict__ grad_angles, T* __restrict__ grad_dihedrals, ChainGeometry geo) {
   enter_after_previous_grid();
   using R = typename ComputeOf<T>::type;
@@ -893,7 +893,7 @@ __global__ void __launch_bounds__(kMaxWarps* kWarp)
 // xyz out and back in between.
 template <typename T>
 __global__ void __launch_bounds__(kMaxWarps* kWarp)
-    block_mse_kernel(BlockArgs<T> args, const T* __restrict__ target, T* __restrict__ loss, T* __restrict__ grad_lengths, T* __restrict__ grad_angles,
+    block_mse_kernel(BlockArgs<T> args, const T* target, T* __restrict__ loss, T* __restrict__ grad_lengths, T* __restrict__ grad_angles,
                      T* __restrict__ grad_dihedrals, ChainGeometry geo) {
   enter_after_previous_grid();
   using R = typename ComputeOf<T>::type;
@@ -1078,7 +1078,7 @@ __device__ __forceinline__ Affine<V> torsion_sweep(const ChainViews<T>& cv, Step
 
 template <typename T>
 __global__ void __launch_bounds__(kMaxWarps* kWarp)
-    torsion_forward_kernel(const T* __restrict__ raw_pairs, int64_t raw_stride, TorsionConsts<typename ComputeOf<T>::type> consts, T* __restrict__ xyz,
+    torsion_forward_kernel(const T* raw_pairs, int64_t raw_stride, TorsionConsts<typename ComputeOf<T>::type> consts, T* __restrict__ xyz,
                            ChainGeometry geo, float* __restrict__ xyz32) {
   enter_after_previous_grid();
   using R = typename ComputeOf<T>::type;
@@ -1264,8 +1264,8 @@ __device__ __forceinline__ void write_pair_grads(const R* X, T* gr, int S, int t
 
 template <typename T>
 __global__ void __launch_bounds__(kMaxWarps* kWarp)
-    torsion_backward_kernel(const T* __restrict__ raw_pairs, int64_t raw_stride, TorsionConsts<typename ComputeOf<T>::type> consts,
-                            const T* __restrict__ grad_xyz, T* __restrict__ grad_raw, int64_t grad_stride, ChainGeometry geo) {
+    torsion_backward_kernel(const T* raw_pairs, int64_t raw_stride, TorsionConsts<typename ComputeOf<T>::type> consts,
+                            const T* grad_xyz, T* __restrict__ grad_raw, int64_t grad_stride, ChainGeometry geo) {
   enter_after_previous_grid();
   using R = typename ComputeOf<T>::type;
   using V = R;
@@ -1305,8 +1305,8 @@ __global__ void __launch_bounds__(kMaxWarps* kWarp)
 // to the recompute form.
 template <typename T>
 __global__ void __launch_bounds__(kMaxWarps* kWarp)
-    torsion_backward_xyz_kernel(const T* __restrict__ raw_pairs, int64_t raw_stride, TorsionConsts<typename ComputeOf<T>::type> consts,
-                                const T* __restrict__ xyz, const T* __restrict__ grad_xyz, T* __restrict__ grad_raw, int64_t grad_stride,
+    torsion_backward_xyz_kernel(const T* raw_pairs, int64_t raw_stride, TorsionConsts<typename ComputeOf<T>::type> consts,
+                                const T* xyz, const T* grad_xyz, T* __restrict__ grad_raw, int64_t grad_stride,
                                 ChainGeometry geo) {
   enter_after_previous_grid();
   using R = typename ComputeOf<T>::type;

@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kMaxWarps* kWarp) long_totals_kernel(BlockArgs
 // xyz of every (chain, segment) from the totals.
 template <typename T>
 __global__ void __launch_bounds__(kMaxWarps* kWarp)
-    long_forward_kernel(BlockArgs<T> args, const typename ComputeOf<T>::type* __restrict__ totals, T* __restrict__ xyz, LongGeometry geo) {
+    long_forward_kernel(BlockArgs<T> args, const typename ComputeOf<T>::type* totals, T* __restrict__ xyz, LongGeometry geo) {
   enter_after_previous_grid();
   using R = typename ComputeOf<T>::type;
   using V = R;
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kMaxWarps* kWarp)
 // (sum g, sum x x g) over each segment's atoms, from the forward's xyz.
 template <typename T>
 __global__ void __launch_bounds__(kMaxWarps* kWarp)
-    long_sums_kernel(const T* __restrict__ xyz, const T* __restrict__ grad_xyz, typename ComputeOf<T>::type* __restrict__ sums, LongGeometry geo) {
+    long_sums_kernel(const T* xyz, const T* grad_xyz, typename ComputeOf<T>::type* __restrict__ sums, LongGeometry geo) {
   enter_after_previous_grid();
   using R = typename ComputeOf<T>::type;
   using V = R;
@@ -249,8 +249,8 @@ __global__ void __launch_bounds__(kMaxWarps* kWarp)
 // its carry from the totals, the force/moment of all later segments from the sums.
 template <typename T>
 __global__ void __launch_bounds__(kMaxWarps* kWarp)
-    long_backward_kernel(BlockArgs<T> args, const typename ComputeOf<T>::type* __restrict__ totals, const typename ComputeOf<T>::type* __restrict__ sums,
-                         const T* __restrict__ grad_xyz, T* __restrict__ grad_lengths, T* __restrict__ grad_angles, T* __restrict__ grad_dihedrals,
+    long_backward_kernel(BlockArgs<T> args, const typename ComputeOf<T>::type* totals, const typename ComputeOf<T>::type* sums,
+                         const T* grad_xyz, T* __restrict__ grad_lengths, T* __restrict__ grad_angles, T* __restrict__ grad_dihedrals,
                          LongGeometry geo) {
   enter_after_previous_grid();
   using R = typename ComputeOf<T>::type;

@@ -457,7 +457,7 @@ struct VecBackwardShared {
 
 template <typename T, int W, bool kPrefetch = false>
 __global__ void __launch_bounds__(kWarp* W)
-    block_backward_xyz_vec_kernel(BlockArgs<T> args, const T* __restrict__ xyz, const T* __restrict__ grad_xyz, T* __restrict__ grad_lengths,
+    block_backward_xyz_vec_kernel(BlockArgs<T> args, const T* xyz, const T* grad_xyz, T* __restrict__ grad_lengths,
                                   T* __restrict__ grad_angles, T* __restrict__ grad_dihedrals, ChainGeometry geo) {
   if constexpr (kPrefetch) {
     if (threadIdx.x == 0) prefetch_point_rows(xyz, grad_xyz, geo, blockIdx.x);  // as block_forward_vec_kernel's
@@ -670,8 +670,8 @@ __global__ void __launch_bounds__(kWarp* W)
 // norm clamp, take the recompute form in the same CTA.
 template <typename T, int W>
 __global__ void __launch_bounds__(kWarp* W)
-    torsion_backward_xyz_vec_kernel(const T* __restrict__ raw_pairs, int64_t raw_stride, TorsionConsts<typename ComputeOf<T>::type> consts,
-                                    const T* __restrict__ xyz, const T* __restrict__ grad_xyz, T* __restrict__ grad_raw, int64_t grad_stride,
+    torsion_backward_xyz_vec_kernel(const T* raw_pairs, int64_t raw_stride, TorsionConsts<typename ComputeOf<T>::type> consts,
+                                    const T* xyz, const T* grad_xyz, T* __restrict__ grad_raw, int64_t grad_stride,
                                     ChainGeometry geo) {
   enter_after_previous_grid();
   static_assert(sizeof(T) >= 4, "vector slots hold 32- and 64-bit types");
@@ -885,7 +885,7 @@ __device__ __forceinline__ void write_grad_slots(const T* X, T* grad_lengths, T*
 // 16-bit recompute form (block_backward_kernel's code) in the same CTA.
 template <typename T, int W>
 __global__ void __launch_bounds__(kWarp* W)
-    block_backward_xyz32_kernel(BlockArgs<T> args, const float* __restrict__ xyz32, const T* __restrict__ grad_xyz, T* __restrict__ grad_lengths,
+    block_backward_xyz32_kernel(BlockArgs<T> args, const float* xyz32, const T* grad_xyz, T* __restrict__ grad_lengths,
                                 T* __restrict__ grad_angles, T* __restrict__ grad_dihedrals, ChainGeometry geo) {
   enter_after_previous_grid();
   static_assert(sizeof(T) == 2, "the float32-position backward serves the 16-bit types");
@@ -1101,8 +1101,8 @@ __host__ __device__ inline size_t torsion_xyz32_bytes(int points, int items) {
 // and clamped pairs take the recompute form (torsion_backward_kernel's) in the same CTA.
 template <typename T, int W>
 __global__ void __launch_bounds__(kWarp* W)
-    torsion_backward_xyz32_kernel(const T* __restrict__ raw_pairs, int64_t raw_stride, TorsionConsts<float> consts, const float* __restrict__ xyz32,
-                                  const T* __restrict__ grad_xyz, T* __restrict__ grad_raw, int64_t grad_stride, ChainGeometry geo) {
+    torsion_backward_xyz32_kernel(const T* raw_pairs, int64_t raw_stride, TorsionConsts<float> consts, const float* xyz32,
+                                  const T* grad_xyz, T* __restrict__ grad_raw, int64_t grad_stride, ChainGeometry geo) {
   enter_after_previous_grid();
   static_assert(sizeof(T) == 2, "the float32-position backward serves the 16-bit types");
   using R = float;

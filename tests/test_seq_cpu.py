@@ -289,3 +289,14 @@ def test_clip_refuses_shared_memory(lib):
     ]
     for arrays in refused:
         assert call(*arrays) == INVALID_VALUE, arrays
+
+
+def test_dependent_kernels_declare_no_input_unchanging():
+    # the same for the kernels of the reconstruction: const with restrict is what allows a read before the wait
+    found = 0
+    for path in (ROOT / "cufk_b200" / "csrc").glob("*.cuh"):
+        for kernel in re.split(r"(?=__global__ )", path.read_text())[1:]:
+            if "enter_after_previous_grid()" in kernel or "wait_for_previous()" in kernel:
+                found += 1
+                assert not re.search(r"const [^,()]*\* __restrict__", kernel.split("{")[0]), path.name
+    assert found >= 10
