@@ -2,6 +2,7 @@
 //
 // As for the reconstruction path: outputs come from the caching allocator on the input's device, launches go to the current
 // stream under a device guard, nothing synchronises with the host, and refusals are RuntimeErrors that name the argument.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -569,6 +570,7 @@ Tensor clip_gradients(const std::vector<Tensor>& grads, double max_norm, double 
     // elements in memory order: any dense layout will do as long as both have the same
     const bool same = g.is_contiguous() ? o.is_contiguous() : (g.is_non_overlapping_and_dense() && g.strides() == o.strides());
     if (!same) {
+      TORCH_CHECK(at::has_internal_overlap(o) != at::MemOverlap::Yes, "an expanded gradient cannot be clipped in place: give it an output of its own");
       from = g.contiguous();
       to = o.is_contiguous() ? o : fresh(g);
       if (!o.is_contiguous()) back.emplace_back(o, to);

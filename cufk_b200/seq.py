@@ -182,6 +182,7 @@ def clip_gradients(grads: Sequence[Tensor], max_norm: float, *, out: Sequence[Te
             when omitted (which are then not written at all where nothing needs clipping).
             A gradient that is listed twice (that of both terms of a sum, say) counts twice in the norm and is scaled once;
             apart from that, what is written for one may not be read or written for another.
+            An expanded gradient (of a sum, say) needs an output of its own.
 
     Returns:
         The norm before clipping, a 0-d tensor on the device: float32, or float64 when some gradient is.  Squares are summed
